@@ -35,8 +35,6 @@ torch::Tensor qkv_prepare(const torch::Tensor& qkv, const torch::Tensor& pos, co
                           double eps);
 std::vector<torch::Tensor> argmax_reduce(const torch::Tensor& val, const torch::Tensor& idx, int64_t n_tiles,
                                          int64_t T);
-void kv_commit(const torch::Tensor& kp, const torch::Tensor& vp, const torch::Tensor& src, const torch::Tensor& dst,
-               int64_t row_elems);
 torch::Tensor attention(const torch::Tensor& q, const torch::Tensor& kc, const torch::Tensor& vc,
                         const torch::Tensor& bt, int64_t page, const torch::Tensor& req, const torch::Tensor& ctx_start,
                         const torch::Tensor& ctx_len, const torch::Tensor& extra, const torch::Tensor& n_extra,
@@ -50,9 +48,9 @@ void kv_write(const torch::Tensor& k, const torch::Tensor& v, const torch::Tenso
               torch::Tensor vc, torch::Tensor ks, torch::Tensor vs);
 std::vector<torch::Tensor> kv_read(const torch::Tensor& kc, const torch::Tensor& vc, const torch::Tensor& ks,
                                    const torch::Tensor& vs, const torch::Tensor& slot, at::ScalarType ty);
-void kv_commit8(const std::vector<torch::Tensor>& k, const std::vector<torch::Tensor>& v,
-                const std::vector<torch::Tensor>& ks, const std::vector<torch::Tensor>& vs, const torch::Tensor& src,
-                const torch::Tensor& dst);
+void kv_commit(const std::vector<torch::Tensor>& k, const std::vector<torch::Tensor>& v,
+               const std::vector<torch::Tensor>& ks, const std::vector<torch::Tensor>& vs, const torch::Tensor& src,
+               const torch::Tensor& dst);
 torch::Tensor attention8(const torch::Tensor& q, const torch::Tensor& kc, const torch::Tensor& vc,
                          const torch::Tensor& ks, const torch::Tensor& vs, const torch::Tensor& bt, int64_t page,
                          const torch::Tensor& req, const torch::Tensor& start, const torch::Tensor& end,
@@ -166,7 +164,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("prepare_axes", &e4::prepare_axes, "q/k norm, multi-axis rotary positions, 16- or 8-bit cache write");
   m.def("kv_write", &e4::kv_write, "quantise K and V rows into an 8-bit cache");
   m.def("kv_read", &e4::kv_read, "read 8-bit cache rows back");
-  m.def("kv_commit8", &e4::kv_commit8);
   m.def("conv_tree", &e4::conv_tree);
   m.def("conv_commit", &e4::conv_commit);
   m.def("conv_commit_scan", &e4::conv_commit_scan);

@@ -255,25 +255,6 @@ __global__ void argmax_reduce_kernel(const float* __restrict__ val, const int* _
   }
 }
 
-// Copy accepted rows' K/V (all attention layers at once): pointers of every layer's cache in ``kp`` / ``vp``.
-__global__ void kv_commit_kernel(const int64_t* __restrict__ kp, const int64_t* __restrict__ vp, int layers,
-                                 const int64_t* __restrict__ src, const int64_t* __restrict__ dst, int n, int row_elems) {
-  pdl_wait();
-  pdl_trigger();
-  const int item = blockIdx.x;  // (layer, move)
-  const int l = item / n, m = item % n;
-  if (l >= layers) return;
-  const int64_t s = src[m], d = dst[m];
-  if (s == d) return;
-  uint4* k = reinterpret_cast<uint4*>(kp[l]);
-  uint4* v = reinterpret_cast<uint4*>(vp[l]);
-  const int vec = row_elems / 8;
-  for (int i = threadIdx.x; i < vec; i += blockDim.x) {
-    k[d * vec + i] = k[s * vec + i];
-    v[d * vec + i] = v[s * vec + i];
-  }
-}
-
 }  // namespace
 
 torch::Tensor gemm_error_word(torch::Device dev);
@@ -366,17 +347,6 @@ std::vector<torch::Tensor> argmax_reduce(const torch::Tensor& val, const torch::
     C10_CUDA_CHECK(launch_pdl(argmax_reduce_kernel, T, 256, 0, at::cuda::getCurrentCUDAStream().stream(), 
         val.data_ptr<float>(), idx.data_ptr<int>(), n_tiles, T, ids.data_ptr<int64_t>(), best.data_ptr<float>()));
   return {ids, best};
-}
-
-void kv_commit(const torch::Tensor& kp, const torch::Tensor& vp, const torch::Tensor& src, const torch::Tensor& dst,
-               int64_t row_elems) {
-  const at::cuda::CUDAGuard g(src.device());
-  const int n = src.size(0), layers = kp.size(0);
-  TORCH_CHECK(row_elems % 8 == 0);
-  if (n && layers)
-    C10_CUDA_CHECK(launch_pdl(kv_commit_kernel, n * layers, 128, 0, at::cuda::getCurrentCUDAStream().stream(), 
-        kp.data_ptr<int64_t>(), vp.data_ptr<int64_t>(), layers, src.data_ptr<int64_t>(), dst.data_ptr<int64_t>(), n,
-        row_elems));
 }
 
 }  // namespace e4

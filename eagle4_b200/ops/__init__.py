@@ -180,6 +180,9 @@ def kv_read(k_cache: QuantKV, v_cache: QuantKV, slots, dtype=torch.bfloat16):
 
 
 def kv_commit(k_caches, v_caches, src_slots, dst_slots):
+    """Move accepted rows ``src_slots[i] -> dst_slots[i]`` in every layer's K and V cache (all 16-bit, or all
+    :class:`QuantKV`). A destination may be an earlier move's source (an accepted path moves down), not a later one's,
+    and no two moves share a destination. A move with a negative slot is skipped."""
     fn = _nat().kv_commit if _cuda(src_slots) else ref.kv_commit
     return fn(k_caches, v_caches, src_slots, dst_slots)
 

@@ -299,9 +299,6 @@ def mamba_commit(xbc, dt_raw, a_log, dt_bias, d_skip, x_pre, state, conv_state, 
     _C.conv_commit(x_pre, conv_state, slots, rows, n_rows, cfg.conv_kernel)
 
 
-_PTRS: Dict[tuple, Tuple[torch.Tensor, torch.Tensor]] = {}
-
-
 def kv_write(k, v, write_slot, k_cache: QuantKV, v_cache: QuantKV) -> None:
     _C.kv_write(k, v, _i64(write_slot), k_cache.data, v_cache.data, k_cache.scale, v_cache.scale)
 
@@ -310,26 +307,17 @@ def kv_read(k_cache: QuantKV, v_cache: QuantKV, slots, dtype):
     return tuple(_C.kv_read(k_cache.data, v_cache.data, k_cache.scale, v_cache.scale, _i64(slots), dtype))
 
 
-def _kv_commit8(k_caches, v_caches, src_slots, dst_slots):
-    if not all(same_form(k, v) for k, v in zip(k_caches, v_caches)):
-        raise TypeError("kv_commit moves rows of caches of one form")
-    _C.kv_commit8([c.data for c in k_caches], [c.data for c in v_caches], [c.scale for c in k_caches],
-                  [c.scale for c in v_caches], src_slots.long().contiguous(), dst_slots.long().contiguous())
-
-
 def kv_commit(k_caches, v_caches, src_slots, dst_slots):
-    if src_slots.numel() == 0:
+    if src_slots.numel() == 0 or not len(k_caches):
         return
-    if isinstance(k_caches[0], QuantKV):
-        return _kv_commit8(k_caches, v_caches, src_slots, dst_slots)
-    key = tuple(t.data_ptr() for t in k_caches)
-    if key not in _PTRS:
-        dev = src_slots.device
-        _PTRS[key] = (torch.tensor([t.data_ptr() for t in k_caches], dtype=torch.int64, device=dev),
-                      torch.tensor([t.data_ptr() for t in v_caches], dtype=torch.int64, device=dev))
-    kp, vp = _PTRS[key]
-    row = k_caches[0].shape[1] * k_caches[0].shape[2]
-    _C.kv_commit(kp, vp, src_slots.long().contiguous(), dst_slots.long().contiguous(), row)
+    forms = {same_form(k, v) for k, v in zip(k_caches, v_caches)}
+    if len(forms) != 1:
+        raise TypeError("kv_commit moves rows of caches of one form")
+    k, v, ks, vs = list(k_caches), list(v_caches), [], []
+    if forms.pop():
+        k, ks = zip(*k)
+        v, vs = zip(*v)
+    _C.kv_commit(k, v, ks, vs, src_slots.long().contiguous(), dst_slots.long().contiguous())
 
 
 # draft head -------------------------------------------------------------------------------------------------------

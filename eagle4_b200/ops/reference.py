@@ -455,9 +455,10 @@ def mamba_commit(xbc, dt_raw, a_log, dt_bias, d_skip, x_pre, state, conv_state, 
 
 # ----------------------------------------------------------------------------------------------- KV commit
 def kv_commit(k_caches, v_caches, src_slots: torch.Tensor, dst_slots: torch.Tensor) -> None:
-    """Move accepted tree rows' K/V to their chain positions in every attention layer (in list order)."""
+    """Move accepted tree rows' K/V to their chain positions in every attention layer (in list order). A move with a
+    negative slot is skipped."""
     src, dst = src_slots.long(), dst_slots.long()
-    keep = src != dst
+    keep = (src != dst) & (src >= 0) & (dst >= 0)
     src, dst = src[keep], dst[keep]
     for cache in list(k_caches) + list(v_caches):
         for s, t in zip(src.tolist(), dst.tolist()):
