@@ -606,6 +606,7 @@ __global__ void __launch_bounds__(num_threads(KB), KB == 1 && NH <= 8 ? 2 : 1) a
       const bool all = __all_sync(0xffffffffu, slot >= 0);
       w.next(p);
       if (i + 1 < count) look();  // the next chunk's entries arrive while this one's copies are issued
+      __syncwarp();  // the lanes' cells are written before others read them
       int64_t src[kPass];
 #pragma unroll
       for (int n = 0; n < kPass; n += 4) {
