@@ -132,6 +132,15 @@ E4_DEV uint64_t sdesc_mn8(uint32_t saddr) {
   return d;
 }
 
+// True in one lane of a converged warp. The issue loop's thread is chosen by this, not by its lane number: the compiler
+// then knows that one lane runs, and products inside data-dependent branches stay right (chosen by ``lane == 0``, a
+// condition around each product gave wrong sums).
+E4_DEV bool elect_one() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(on));
+  return on != 0;
+}
+
 // D[tmem] (+)= A[smem] . B[smem]^T on 8-bit operands: e4m3 with fp32 sums, or int8 with int32 sums.
 template <int FMT>
 E4_DEV void umma8(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -139,12 +148,12 @@ E4_DEV void umma8(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint3
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
   else
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // Instruction descriptor: e4m3 x e4m3 -> fp32, or s8 x s8 -> s32; ``a_mn``: A is MN-major.
 template <int FMT>
@@ -511,7 +520,7 @@ __global__ void __launch_bounds__(num_threads(KB), KB == 1 && NH <= 8 ? 2 : 1) a
     // ---- MMAs, by one thread: S(i + 1) before O(i) where both have the same query. Waiting for w_full(i) also says that
     // S(i) and its scales have been read and O(i - 2) folded, so the buffers of S(i + 2) and O(i) are free. Head dims
     // past D are zeros in both operands: all products are issued, whatever D is.
-    if (lane == 0) {
+    if (elect_one()) {
       tc_fence_after();
       const uint32_t tmem = tmem_holder, id_s = idesc8<FMT>(NC, false), id_o = idesc8<FMT>(NC, true);
       const uint32_t kt = smem_u32(smem), vt = smem_u32(Vs), qt = smem_u32(Qt), wt = smem_u32(Ws);
