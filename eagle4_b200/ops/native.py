@@ -7,7 +7,6 @@ Importing this module on a machine with a GPU loads the extension; if it cannot 
 from __future__ import annotations
 
 import contextlib
-import functools
 import math
 from typing import Dict, Optional, Tuple
 
@@ -187,12 +186,17 @@ def rope_tables(rot: int, theta: float, device, max_pos: int = 1 << 17) -> Tuple
     return _ROPE[key]
 
 
-@functools.lru_cache(maxsize=64)
+_TURNS: Dict[tuple, torch.Tensor] = {}  # never evicted: captured graphs keep the tables' addresses
+
+
 def rope_turns(rot: int, theta: float, device: torch.device) -> torch.Tensor:
     """Turns per position of every rotary frequency, ``theta^(-i/half) / 2 pi`` in float64 ``[half]``."""
-    half = max(rot // 2, 1)
-    inv = 1.0 / (theta ** (torch.arange(0, half, dtype=torch.float64) / half))
-    return (inv / (2 * math.pi)).to(device)
+    key = (rot, theta, str(device))
+    if key not in _TURNS:
+        half = max(rot // 2, 1)
+        inv = 1.0 / (theta ** (torch.arange(0, half, dtype=torch.float64) / half))
+        _TURNS[key] = (inv / (2 * math.pi)).to(device)
+    return _TURNS[key]
 
 
 def _prepare_axes(qkv, cfg, pos, write_slot, k_cache, v_cache, q_norm, k_norm):
