@@ -523,7 +523,7 @@ torch::Tensor prepare_axes(const torch::Tensor& qkv, const torch::Tensor& pos, c
   TORCH_CHECK(qkv.size(1) == (Hq * (gated ? 2 : 1) + 2 * Hk) * D, who,
               ": the projection's columns do not match the heads");
   TORCH_CHECK(rot >= 0 && rot % 2 == 0 && rot <= D && inv.numel() >= rot / 2, who, ": rotary dims must be even, up to the head dim");
-  TORCH_CHECK(pos.dim() == 2 && pos.size(1) == T && pos.scalar_type() == at::kLong && pos.stride(1) == 1 &&
+  TORCH_CHECK(pos.dim() == 2 && pos.size(1) == T && pos.scalar_type() == at::kLong && (pos.stride(1) == 1 || T == 1) &&
                   pos.size(0) >= 1 && pos.size(0) <= kMaxAxes && int64_t(sections.size()) == pos.size(0),
               who, ": positions must be int64 [axes, T], one section per axis, up to 4 axes");
   TORCH_CHECK(slot.dim() == 1 && slot.size(0) == T && slot.scalar_type() == at::kLong && slot.is_contiguous(), who,

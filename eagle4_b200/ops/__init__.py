@@ -79,8 +79,8 @@ def concat_norms(e, h, we, wh, eps: float) -> torch.Tensor:
 def qkv_prepare(qkv, cfg, pos, write_slot, k_cache, v_cache, q_norm, k_norm):
     """Split the fused projection, apply q / k norms and rotary positions, write K and V at ``write_slot`` and return
     ``(q, gate)``. The caches are 16-bit tensors or :class:`QuantKV` (rows are quantised as they are written).
-    ``pos [T]``, or ``pos [axes, T]`` with ``cfg.rope_sections`` / ``cfg.rope_interleaved`` (time, height and width of
-    image and video tokens; the layout is in ``ops.quant.rope_layout``). With 8-bit caches or several axes a row with a
+    ``pos [T]`` (or ``[1, T]``), or ``pos [axes, T]`` with ``cfg.rope_sections`` / ``cfg.rope_interleaved`` (time, height
+    and width of image and video tokens; the layout is in ``ops.quant.rope_layout``). With 8-bit caches or several axes a row with a
     negative slot is not written."""
     if _cuda(qkv):
         return _nat().qkv_prepare(qkv, cfg, pos, write_slot, k_cache, v_cache, q_norm, k_norm)

@@ -211,14 +211,16 @@ def _prepare_axes(qkv, cfg, pos, write_slot, k_cache, v_cache, q_norm, k_norm):
     quant = isinstance(k_cache, QuantKV)
     k, ks = k_cache if quant else (k_cache, _NONE)
     v, vs = v_cache if quant else (v_cache, _NONE)
-    q = _C.prepare_axes(rows, pos if pos.stride(-1) == 1 else pos.contiguous(), _i64(write_slot), k, v, ks, vs, q_norm, k_norm, bool(cfg.norm_offset),
-                        rope_turns(cfg.rotary_dim, cfg.rope_theta, qkv.device), list(sections), interleaved,
-                        cfg.num_heads, cfg.rotary_dim, bool(cfg.attn_output_gate), float(cfg.rms_norm_eps))
+    q = _C.prepare_axes(rows, pos if pos.stride(-1) == 1 else pos.contiguous(), _i64(write_slot), k, v, ks, vs, q_norm,
+                        k_norm, bool(cfg.norm_offset), rope_turns(cfg.rotary_dim, cfg.rope_theta, qkv.device),
+                        list(sections), interleaved, cfg.num_heads, cfg.rotary_dim, bool(cfg.attn_output_gate), float(cfg.rms_norm_eps))
     hd = cfg.num_heads * cfg.head_dim
     return q, qkv[:, hd: 2 * hd] if cfg.attn_output_gate else None
 
 
 def qkv_prepare(qkv, cfg, pos, write_slot, k_cache, v_cache, q_norm, k_norm):
+    if pos.dim() == 2 and pos.shape[0] == 1:  # one axis
+        pos = pos[0]
     if same_form(k_cache, v_cache) or pos.dim() == 2:
         return _prepare_axes(qkv, cfg, pos, write_slot, k_cache, v_cache, q_norm, k_norm)
     cos_t, sin_t = rope_tables(cfg.rotary_dim, cfg.rope_theta, qkv.device)

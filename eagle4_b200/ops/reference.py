@@ -128,6 +128,8 @@ def qkv_prepare(qkv: torch.Tensor, cfg, pos: torch.Tensor, write_slot: torch.Ten
     or positions of several axes (``pos [axes, T]``) the norm and the rotation are rounded once, as they are stored,
     and a row with a negative slot is not written.
     """
+    if pos.dim() == 2 and pos.shape[0] == 1:  # one axis
+        pos = pos[0]
     if same_form(k_cache, v_cache) or pos.dim() == 2:
         return _qkv_prepare_axes(qkv, cfg, pos, write_slot, k_cache, v_cache, q_norm, k_norm)
     t = qkv.shape[0]
