@@ -51,9 +51,10 @@ namespace {
 constexpr int kChunk = 128;    // logical keys per chunk: the MMA's M
 constexpr int kLoad = 128;     // threads that load
 // Threads for softmax and output, before the loading ones and the warp that issues the MMAs (an issue takes some 90
-// cycles, too much for a warp the others wait for): one group of 128 up to head dim 128, where two CTAs share an SM;
-// two with half of the heads each above, where one CTA has the SM and a chunk's output is twice as long. Measured: two
-// groups at head dim 128 need 500 us for 32 x 32768 keys where one needs 400 (twice the waiting threads, the same work).
+// cycles, too much for a warp the others wait for): one group of 128 up to head dim 128, where two CTAs share an SM (up
+// to 8 heads); two with half of the heads each above, where one CTA has the SM and a chunk's output is twice as long.
+// Measured when it was tried: two groups at head dim 128 need 500 us for 32 x 32768 keys where one needed 400 (twice the
+// waiting threads, the same work).
 __host__ __device__ constexpr int math_threads(int KB) { return KB * 128; }
 __host__ __device__ constexpr int num_threads(int KB) { return math_threads(KB) + kLoad + 32; }
 constexpr int kTerms = 3;      // 8-bit digits per 16-bit query or weight
@@ -234,9 +235,14 @@ E4_DEV float pow2f(int e) { return __int_as_float((e + 127) << 23); }
 constexpr int kStages = 3;
 __host__ __device__ constexpr int columns(int NH) { return (kTerms * NH + 15) / 16 * 16; }
 __host__ __device__ constexpr int smem_bytes(int KB, int NH) {
-  // tiles start on 1024 bytes: K and V tiles, then Q [KB][columns][128], two W [columns][128], then the scales
-  return 1024 + kStages * (2 * KB * kChunk * 128 + 2 * kChunk * 4) + (KB + 2) * columns(NH) * 128;
+  // from a 1024-byte boundary on: K and V tiles, then Q [KB][columns][128], two W [columns][128], then the scales
+  return kStages * (2 * KB * kChunk * 128 + 2 * kChunk * 4) + (KB + 2) * columns(NH) * 128;
 }
+// CTAs that share an SM: two need 2 x (dynamic + 2048 static + 1024 reserved) bytes within its 228 KB and 96 registers a
+// thread. With 5 to 8 heads the two fit to the byte and spill some 200 bytes a thread: 32 rows of 32768 keys, 64/8 heads x
+// 128, take 671 us (fp8) and 664 us (int8), one CTA without spills 642 and 768.
+__host__ __device__ constexpr int ctas_per_sm(int KB, int NH) { return KB == 1 && NH <= 8 ? 2 : 1; }
+static_assert(ctas_per_sm(1, 8) * (smem_bytes(1, 8) + 2048 + 1024) <= 228 * 1024, "two CTAs an SM up to 8 heads");
 // S and O accumulators, two of each
 __host__ __device__ constexpr int tmem_columns(int KB, int NH) {
   int n = 32;
@@ -405,10 +411,10 @@ E4_DEV void end_piece(const Args& p, const Walk& f, State<H, KB>& s, int g0, int
 
 // ------------------------------------------------------------------------------------------------------- kernel
 template <int FMT, int NH, int KB>
-__global__ void __launch_bounds__(num_threads(KB), KB == 1 && NH <= 8 ? 2 : 1) attn8_kernel(const Args p) {
+__global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_kernel(const Args p) {
   constexpr int NC = columns(NH), NS = kStages, kTile = kChunk * 128, kTmem = tmem_columns(KB, NH);
   constexpr int kMath = math_threads(KB), kThreads = num_threads(KB), H = NH / KB;  // H: heads per thread
-  extern __shared__ unsigned char smem_raw[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ uint64_t k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], q_full, w_full[2], s_done[2], o_done[2];
   __shared__ uint32_t tmem_holder;
   __shared__ int s_warp[kThreads / 32], s_at[2][4];  // begin and end: row, head, chunk, position
@@ -416,7 +422,6 @@ __global__ void __launch_bounds__(num_threads(KB), KB == 1 && NH <= 8 ? 2 : 1) a
   __shared__ __align__(16) int s_cell[kLoad / 32][32];
   __shared__ int s_bad;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char* Vs = smem + NS * KB * kTile;
   unsigned char* Qt = smem + NS * 2 * KB * kTile;
   unsigned char* Ws = Qt + KB * NC * 128;
@@ -872,11 +877,11 @@ void launch(Args p, int64_t bound, const torch::Tensor& q, cudaStream_t stream) 
     C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_set[dev] = true;
   }
-  const int full = at::cuda::getCurrentDeviceProperties()->multiProcessorCount * (KB == 1 && NH <= 8 ? 2 : 1);
+  const int full = at::cuda::getCurrentDeviceProperties()->multiProcessorCount * ctas_per_sm(KB, NH);
   const int grid = int(std::min<int64_t>(bound, full));
   p.spread = full;
-  // (two CTAs an SM where registers and shared memory allow: up to head dim 128 and 8 heads.) A CTA's pieces of one (row,
-  // kv head) are at most its share of chunks (its bounds move by less than a piece), and at most all of the row's.
+  // A CTA's pieces of one (row, kv head) are at most its share of chunks (its bounds move by less than a piece), and at
+  // most all of the row's.
   const int64_t most = std::min<int64_t>(p.max_chunks, ceil_div(full, p.Hk) + 1);
   p.area = int(std::min<int64_t>(2 * ceil_div(bound, grid) + 1, most));
   const int64_t info = grid * 4;
