@@ -67,7 +67,7 @@ struct Args {
   const int *bt, *req, *start, *end, *extra, *n_extra;
   const void* gate;
   void* out;
-  float* ws;    // partials: [CTA][2 areas][slots][G][D + 4]
+  float* ws;    // partials: [CTA boundary][piece][G][D + 4]; a (row, kv head) lies with the first boundary that cuts it
   int4* info;   // per CTA: (row, head, piece, the row's chunks) where its work begins (an empty one: the next one's)
   int* err;
   int64_t slots, ldg;
@@ -345,7 +345,7 @@ E4_DEV float warp_sums(float* v, int lane) {
 template <int H, int KB>
 struct State {
   float gM[H], gL[H], gA[KB][H], rM[H], rL[H], rA[KB][H];
-  int part, area, in_piece;
+  int region, part, in_piece;  // where its partials go: the first boundary that cuts it (less one), the piece
   bool whole;  // this CTA holds all of the row's chunks
   E4_DEV void clear_piece() {
     in_piece = 0;
@@ -372,10 +372,10 @@ struct State {
 template <int H, int KB>
 E4_DEV void end_piece(const Args& p, const Walk& f, State<H, KB>& s, int g0, int t, bool last) {
   if (!s.whole) {
-    if (s.part >= p.area) {
+    if (s.part >= p.area || s.region + 1 >= gridDim.x) {
       record_error(p.err, kErrBadShape);
     } else {
-      float* ws = p.ws + (((size_t(blockIdx.x) * 2 + s.area) * p.area + s.part) * p.G + g0) * (p.D + 4);
+      float* ws = p.ws + ((size_t(s.region) * p.area + s.part) * p.G + g0) * (p.D + 4);
 #pragma unroll
       for (int g = 0; g < H; ++g) {
         if (g0 + g >= p.G) break;
@@ -664,6 +664,9 @@ __global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_ke
     float m[H], pm[H];  // maxima of this chunk and the one before
     // One step takes chunk i to its weights, then folds the output of chunk i - 1, whose product ran meanwhile.
     Walk f = w;  // the chunk being folded
+    // The boundary before CTA b lies at chunk floor(chunks b / grid): the first one past the start of the (row, kv head)
+    // that this CTA begins inside of.
+    const int first_cut = w.c ? int((int64_t(s_at[0][3] - w.c + 1) * gridDim.x + chunks - 1) / chunks) - 1 : 0;
     for (int i = 0; i <= count; ++i) {
       const int st = i % NS;
       if (i < count) {
@@ -761,8 +764,8 @@ __global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_ke
         const int j = i - 1;
         if (j == 0 || f.c == 0) {
           s.whole = f.c == 0 && f.n <= count - j;
-          s.part = 0;
-          s.area = j == 0 ? 0 : 1;
+          s.part = f.c / f.piece;
+          s.region = f.c == 0 ? blockIdx.x : first_cut;
           s.clear_piece();
           s.clear_row();
         }
@@ -805,12 +808,11 @@ __global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_ke
 }
 
 // Folds the (row, kv head)s that a CTA boundary cut: block (i, g) takes the one that CTA i begins inside of, if no
-// earlier boundary cuts it, and query head g of its group; thread t holds head dim t. The pieces' places and statistics
-// are gathered by all threads first, so that the fold, a chain of one fused multiply-add per piece, waits for one
-// load latency per kMergeBatch pieces.
+// earlier boundary cuts it, and query head g of its group; thread t holds head dim t. All threads fetch the pieces'
+// statistics first, so that the fold, a chain of one fused multiply-add per piece, waits for one load latency per
+// kMergeBatch pieces.
 constexpr int kMergeBatch = 16, kMaxPieces = 512;
-__global__ void __launch_bounds__(256) attn8_merge_kernel(const Args p, int grid) {
-  __shared__ int place[kMaxPieces];
+__global__ void __launch_bounds__(256) attn8_merge_kernel(const Args p) {
   __shared__ float2 stat[kMaxPieces];
   pdl_wait();
   pdl_trigger();
@@ -818,37 +820,23 @@ __global__ void __launch_bounds__(256) attn8_merge_kernel(const Args p, int grid
   const int4 at = p.info[i], prev = p.info[i - 1];
   const int r = at.x, h = at.y;
   if (r >= p.T || at.z == 0) return;
-  const bool same = prev.x == r && prev.y == h;
-  if (same && prev.z > 0) return;
+  if (prev.x == r && prev.y == h && prev.z > 0) return;
   const int n = at.w, ps = piece_chunks(p, n), pieces = (n + ps - 1) / ps;
-  if (pieces > kMaxPieces) {
+  if (pieces > kMaxPieces || pieces > p.area) {
     record_error(p.err, kErrBadShape);
     return;
   }
-  // CTA c holds pieces [where it begins, where c + 1 does); only CTA i - 1 may hold other work before them
-  for (int c = i - 1 + d; c < grid; c += blockDim.x) {
-    const int4 b0 = c < i ? make_int4(r, h, 0, 0) : p.info[c];
-    if (b0.x != r || b0.y != h) break;
-    int stop = pieces;
-    if (c + 1 < grid) {
-      const int4 b1 = p.info[c + 1];
-      if (b1.x == r && b1.y == h) stop = b1.z;
-    }
-    const int area = c < i && !same ? 1 : 0;
-    for (int j = b0.z; j < stop; ++j) place[j] = (c * 2 + area) * p.area + (j - b0.z);
-  }
-  __syncthreads();
   const int stride = p.G * (p.D + 4);
-  const float* ws = p.ws + g * (p.D + 4);
+  const float* ws = p.ws + size_t(blockIdx.x) * p.area * stride + g * (p.D + 4);
   float a[kMergeBatch];
   auto fetch = [&](int j0) {
 #pragma unroll
     for (int j = 0; j < kMergeBatch; ++j)
-      a[j] = j0 + j < pieces && d < p.D ? __ldcg(ws + size_t(place[j0 + j]) * stride + d) : 0.f;
+      a[j] = j0 + j < pieces && d < p.D ? __ldcg(ws + size_t(j0 + j) * stride + d) : 0.f;
   };
   fetch(0);  // in flight with the statistics
   for (int j = d; j < pieces; j += blockDim.x) {
-    const float* x = ws + size_t(place[j]) * stride + p.D;
+    const float* x = ws + size_t(j) * stride + p.D;
     stat[j] = make_float2(__ldcg(x), __ldcg(x + 1));
   }
   __syncthreads();
@@ -880,16 +868,14 @@ void launch(Args p, int64_t bound, const torch::Tensor& q, cudaStream_t stream) 
   const int full = at::cuda::getCurrentDeviceProperties()->multiProcessorCount * ctas_per_sm(KB, NH);
   const int grid = int(std::min<int64_t>(bound, full));
   p.spread = full;
-  // A CTA's pieces of one (row, kv head) are at most its share of chunks (its bounds move by less than a piece), and at
-  // most all of the row's.
-  const int64_t most = std::min<int64_t>(p.max_chunks, ceil_div(full, p.Hk) + 1);
-  p.area = int(std::min<int64_t>(2 * ceil_div(bound, grid) + 1, most));
+  // a boundary's room: all pieces of one (row, kv head)
+  p.area = int(std::min<int64_t>(p.max_chunks, ceil_div(full, p.Hk)));
   const int64_t info = grid * 4;
-  auto ws = torch::empty({info + int64_t(grid) * 2 * p.area * p.G * (p.D + 4)}, q.options().dtype(torch::kFloat32));
+  auto ws = torch::empty({info + int64_t(grid - 1) * p.area * p.G * (p.D + 4)}, q.options().dtype(torch::kFloat32));
   p.info = reinterpret_cast<int4*>(ws.data_ptr<float>());
   p.ws = ws.data_ptr<float>() + info;
   C10_CUDA_CHECK(launch_pdl(kernel, grid, num_threads(KB), smem, stream, p));
-  if (grid > 1) C10_CUDA_CHECK(launch_pdl(attn8_merge_kernel, dim3(grid - 1, p.G), p.D <= 128 ? 128 : 256, 0, stream, p, grid));
+  if (grid > 1) C10_CUDA_CHECK(launch_pdl(attn8_merge_kernel, dim3(grid - 1, p.G), p.D <= 128 ? 128 : 256, 0, stream, p));
 }
 
 }  // namespace

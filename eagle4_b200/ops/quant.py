@@ -79,6 +79,16 @@ def same_form(k_cache: Cache, v_cache: Cache) -> bool:
     return k8
 
 
+def attention_workspace(rows: int, q_heads: int, kv_heads: int, dim: int, max_keys: int, sms: int = 148) -> int:
+    """Bytes that ``ops.attention`` over 8-bit caches allocates beside its output while it runs: the partial sums of the
+    (row, kv head)s that its blocks' bounds cut, up to one at each bound, and where each block begins."""
+    group = q_heads // kv_heads
+    blocks = sms * (2 if dim <= 128 and group <= 8 else 1)
+    chunks = max(1, -(-max_keys // 128))
+    grid = min(rows * kv_heads * chunks, blocks)
+    return 4 * (4 * grid + (grid - 1) * min(chunks, -(-blocks // kv_heads)) * group * (dim + 4)) if rows else 0
+
+
 def rope_layout(cfg, pos: torch.Tensor) -> Tuple[Tuple[int, ...], bool]:
     """How the rows' positions turn the rotary frequencies: ``(sections, interleaved)``.
 

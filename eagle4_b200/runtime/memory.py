@@ -6,7 +6,9 @@ cache and recurrent states, the draft's KV cache. Everything scales with the KV 
 the per-request states, so the plan also answers the largest ``kv_tokens`` that fits a memory budget (the server's
 ``--kv-tokens``). ``prefill`` estimates the largest transient of a prefill: one piece of ``prefill_chunk`` rows
 through the widest projection plus a few hidden-size buffers, and the aux hidden states of a whole ``max_len``
-prompt kept for the draft. ``reserve_gb`` stands for what the plan does not count: decode activations, CUDA graph
+prompt kept for the draft. ``attention`` is the workspace of attention over an 8-bit KV cache, once for prefill and once
+in the graphs' pool (hundreds of MB where a rank holds few kv heads; 0 with a 16-bit cache, whose attention's workspace
+the plan does not count). ``reserve_gb`` stands for what the plan does not count: decode activations, CUDA graph
 pools, the tensor-parallel buffers, the CUDA context (a few GB at the flagship shapes; measure with
 ``torch.cuda.mem_get_info`` on the target GPU for a tighter figure).
 """
@@ -30,6 +32,7 @@ class MemoryPlan:
     kv_tokens: int
     reserve: int
     prefill: int = 0         # bytes of the largest prefill transient (one piece's activations, the prompt's aux rows)
+    attention: int = 0       # bytes of the 8-bit cache's attention workspaces (prefill, decode graphs)
 
     @property
     def kv(self) -> int:
@@ -37,11 +40,11 @@ class MemoryPlan:
 
     @property
     def total(self) -> int:
-        return self.weights + self.kv + self.state_bytes + self.reserve + self.prefill
+        return self.weights + self.kv + self.state_bytes + self.reserve + self.prefill + self.attention
 
     def kv_tokens_within(self, budget_bytes: float) -> int:
         """The largest KV token budget (a multiple of 1024) whose plan fits ``budget_bytes``."""
-        free = budget_bytes - self.weights - self.state_bytes - self.reserve - self.prefill
+        free = budget_bytes - self.weights - self.state_bytes - self.reserve - self.prefill - self.attention
         return max(0, int(free // self.kv_bytes_per_token) // 1024 * 1024)
 
     def summary(self, budget_gb: Optional[float] = None) -> Dict[str, float]:
@@ -71,7 +74,7 @@ def plan(target_cfg, draft_cfg=None, *, tp: int = 1, max_batch: int = 1, max_len
     from eagle4_b200.models import weights
     from eagle4_b200.models.draft import DraftCache
     from eagle4_b200.models.target import TargetCache
-    from eagle4_b200.ops.quant import cache_tensors, kv_code
+    from eagle4_b200.ops.quant import attention_workspace, cache_tensors, kv_code
     from eagle4_b200.parallel.sharding import shard_draft, shard_target
 
     meta = torch.device("meta")
@@ -97,5 +100,9 @@ def plan(target_cfg, draft_cfg=None, *, tp: int = 1, max_batch: int = 1, max_len
     hidden = target_cfg.hidden_size
     aux = len(draft_cfg.aux_layer_ids) * hidden if draft_cfg is not None else 0
     prefill = (min(prefill_chunk, max_len) * (widest + 4 * hidden) + max_len * aux) * esize
+    attention = 0
+    if kv_code(kv_dtype) is not None and one.k:
+        attention = sum(attention_workspace(rows, ltc.num_heads, ltc.num_kv_heads, ltc.head_dim, row_len)
+                        for rows in (min(prefill_chunk, max_len), max_batch * verify))
     return MemoryPlan(weights=w_bytes, kv_bytes_per_token=kv_page // page, state_bytes=state,
-                      kv_tokens=int(tokens), reserve=int(reserve_gb * GB), prefill=int(prefill))
+                      kv_tokens=int(tokens), reserve=int(reserve_gb * GB), prefill=int(prefill), attention=attention)
