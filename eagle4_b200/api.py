@@ -19,6 +19,7 @@ from eagle4_b200.core.config import HarnessConfig, parse_harness_config
 from eagle4_b200.models import configs, weights
 from eagle4_b200.models.draft import DraftModel
 from eagle4_b200.models.target import TargetModel
+from eagle4_b200.ops.quant import kv_code
 from eagle4_b200.runtime.engine import Engine
 
 NAMED = {
@@ -56,7 +57,8 @@ class LLM:
         ``kv_dtype``: ``"fp8"`` or ``"int8"`` holds the target's KV cache in 8 bits (None or ``"bf16"``: 16 bits)."""
         if isinstance(config, str):
             config = parse_harness_config(config)
-        config = _with_packaged_profile(config, target, draft)
+        if kv_code(kv_dtype) is None:  # (the packaged profiles are measured over 16-bit caches)
+            config = _with_packaged_profile(config, target, draft)
         self.target, self.draft, self.tree = target, draft, tree
         self.engine = Engine(target, draft, max_reqs=max_batch, max_len=max_len, page=page, steps=tree.steps,
                              top_k=tree.top_k, verify_tokens=tree.draft_tokens, config=config,

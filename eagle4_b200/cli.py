@@ -66,6 +66,8 @@ def serve_config(output: Path) -> dict:
 def _serve_command(args) -> str:
     serve = ["--model", args.model] + (["--draft", args.draft] if args.draft else []) + \
         ["--config", json.dumps(serve_config(args.output))]
+    if args.kv_dtype != "bf16":
+        serve += ["--kv-dtype", args.kv_dtype]
     if args.tp > 1:
         launch = ["python", "-m", "torch.distributed.run", "--nnodes", "1", "--nproc-per-node", str(args.tp),
                   "--master-addr", "127.0.0.1", "-m", "eagle4_b200.serve"]
@@ -79,7 +81,8 @@ def _worker_args(args) -> List[str]:
     out = ["calibrate", "--model", args.model, "--output", str(args.output), "--tp", str(args.tp), "--worker",
            "--batch-sizes", ",".join(map(str, args.batch_sizes)), "--context-step", str(args.context_step),
            "--context-stop", str(args.context_stop), "--repeats", str(args.repeats), "--steps", str(args.steps),
-           "--top-k", str(args.top_k), "--draft-tokens", str(args.draft_tokens), "--kind", args.kind]
+           "--top-k", str(args.top_k), "--draft-tokens", str(args.draft_tokens), "--kind", args.kind,
+           "--kv-dtype", args.kv_dtype]
     if args.draft:
         out += ["--draft", args.draft]
     if args.package:
@@ -93,15 +96,15 @@ def _measure(args, tp=None) -> dict:
     import torch
 
     from eagle4_b200.api import TreeSpec
-    from eagle4_b200.core.live_costs import CostKey
+    from eagle4_b200.core.live_costs import CostKey, key_dtype
     from eagle4_b200.runtime.calibrate import calibrate
 
     world, rank = (tp.world, tp.rank) if tp is not None else (1, 0)
     tree = TreeSpec(args.steps, 1 if args.kind == "chain" else args.top_k, args.draft_tokens)
     llm = build_llm(args.model, args.draft, max_batch=max(args.batch_sizes), max_len=args.context_stop + 256,
-                    tree=tree, tp=tp)
+                    tree=tree, tp=tp, kv_dtype=args.kv_dtype)
     key = CostKey(gpu=torch.cuda.get_device_name(), gpu_count=world, model=args.model, draft=str(args.draft or ""),
-                  engine="eagle4_b200", dtype="bfloat16")
+                  engine="eagle4_b200", dtype=key_dtype(args.kv_dtype))
     if args.kind == "chain":
         from eagle4_b200.runtime.calibrate import calibrate_chain
 
@@ -216,6 +219,8 @@ def _calibrate(args) -> int:
     import torch
 
     args.output = (args.output or Path("eagle4-calibration")).resolve()
+    if args.package and args.kv_dtype != "bf16":
+        raise ValueError("packaged profiles are matched without the KV cache's form: --package needs --kv-dtype bf16")
     if args.worker:
         return _calibrate_worker(args)
     if args.tp > 1:
@@ -302,6 +307,8 @@ def main(argv: Optional[List[str]] = None) -> int:
     cal.add_argument("--draft-tokens", type=_positive, default=16)
     cal.add_argument("--kind", choices=("tree", "chain"), default="tree",
                      help="tree: cost tables from timed forwards; chain: served chain rounds and acceptance")
+    cal.add_argument("--kv-dtype", choices=("bf16", "fp8", "int8"), default="bf16",
+                     help="the server's --kv-dtype: the KV cache whose attention is timed")
     cal.add_argument("--dry-run", action="store_true", help="print settings and the serving command only")
     cal.add_argument("--package", action="store_true",
                      help="also write profile.json so the directory can ship as a packaged cost profile")

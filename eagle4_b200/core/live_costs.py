@@ -100,6 +100,24 @@ def check_key(data_path: str, key: CostKey) -> None:
         )
 
 
+def key_dtype(kv_dtype: Optional[str] = None) -> str:
+    """A key's ``dtype`` of this package's engine: the weights' type, and the KV cache's where it is not theirs."""
+    return "bfloat16" if kv_dtype in (None, "bf16") else f"bfloat16+kv_{kv_dtype}"
+
+
+def check_kv_form(data_path: str, kv_dtype: Optional[str]) -> bool:
+    """Whether tables of this package's engine were measured over this engine's form of KV cache (its attention kernel);
+    warns where not. Unkeyed directories and other engines' pass."""
+    stored = read_key(data_path)
+    if stored is None or stored.engine != "eagle4_b200":
+        return True
+    theirs, ours = stored.dtype.partition("+kv_")[2] or "bf16", kv_dtype or "bf16"
+    if theirs != ours:
+        log.warning("the cost tables under %s were measured over a %s KV cache and this engine's is %s, which another "
+                    "attention kernel reads: calibrate with --kv-dtype %s", data_path, theirs, ours, ours)
+    return theirs == ours
+
+
 @dataclass
 class Cell:
     us: float = 0.0

@@ -161,6 +161,10 @@ class Engine:
                                               pages=kv_pages)
             shape = TreeShape(top_k=top_k, max_depth=steps)
         self.config = config or HarnessConfig(mode=Mode.STATIC)
+        if self.config.data_path and self.config.mode.uses_cost_model:
+            from eagle4_b200.core.live_costs import check_kv_form
+
+            check_kv_form(self.config.data_path, kv_dtype)
         self.policy = RoundPolicy(self.config, top_k=top_k, steps=steps, verify_tokens=verify_tokens,
                                   target_is_moe=target.cfg.is_moe)
         # chain rounds (top-k 1): the width per batch bucket is chosen on served rounds (or a calibrated schedule)
