@@ -7,8 +7,8 @@
 //
 // The codes go to the tensor cores as they lie in the cache; no 8-bit value is ever widened. What is not 8-bit is
 // cut into 8-bit digits instead: q and the weights p_j b_j become three digits each (e4m3: the rounded value, then
-// the remainder times 16, twice, 12 significant bits; int8: signed base-256 digits of a 23-bit fixed-point number), one
-// MMA column per digit, and the three products are added in fp32 afterwards. The tensor cores are idle most of the
+// the remainder times 16, twice: within 2^-12 of the value down to 2^-14 of full scale, within 2^-26 of full scale below;
+// int8: signed base-256 digits of a fixed-point number, within 2^-23 of full scale), one MMA column per digit, and the three products are added in fp32 afterwards. The tensor cores are idle most of the
 // time at these sizes, so three columns cost nothing, and the operands need half the shared memory and no conversion
 // work per key. The value scale goes into the softmax: u_j = score_j log2(e) + log2(b_j) is what the running maximum
 // is taken over, so the weights w_j = 2^(u_j - max u) = p_j b_j lie in (0, 1] whatever the scales are, which is what
@@ -28,8 +28,8 @@
 // Bound: HBM for long caches (32 rows of 32768 keys, 8 x 128: 424 us, 5.2 TB/s, 0.80 of the copy rate; one row of 131071
 // keys, 4 x 256 int8: 59 us, 0.71); the softmax warps' instructions, some 2000 cycles a chunk, where rows are short or
 // share their keys through L2 (8 x 16 tree rows over 1900 keys: 126 us); launch and the dependent loads of two kernels
-// for one short row (4096 keys: 14 us). Three digits instead of two cost nothing measurable and keep fp16 outputs at the
-// error of a 32-bit softmax.
+// for one short row (4096 keys: 14 us). Three digits instead of two cost nothing measurable and keep the
+// digits' error at or below the rounding of fp16 outputs.
 //
 // A row's result must not depend on its batch: a token decoded alone and the same token verified inside a tree have to
 // agree bit for bit. So the order of folding is fixed by the row's key count alone: a row's chunks are folded in order
