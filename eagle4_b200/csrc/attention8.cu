@@ -427,7 +427,6 @@ __global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_ke
   unsigned char* Ws = Qt + KB * NC * 128;
   float* scales = reinterpret_cast<float*>(Ws + 2 * NC * 128);  // [stage][K 128 | V 128]
 
-  if (warp == 0) tmem_alloc(&tmem_holder, kTmem);
   if (tid == 32) {
     for (int i = 0; i < NS; ++i) {
       mbar_init(&k_full[i], kLoad);
@@ -449,8 +448,10 @@ __global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_ke
   if (p.D < KB * 128)
     for (int i = tid; i < NS * 2 * KB * kTile / 16; i += kThreads)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  // TMEM is taken after the kernel before has ended and before the next one may start: two kernels on one SM that each
+  // hold some of it, one waiting for the other, would wait for good.
   pdl_wait();
-  pdl_trigger();
+  if (warp == 0) tmem_alloc(&tmem_holder, kTmem);
 
   // chunks of all rows and heads: a block-wide prefix sum, a run of rows per thread
   const int per = (p.T + kThreads - 1) / kThreads;
@@ -469,6 +470,7 @@ __global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_ke
     s_at[tid][3] = -1;
   }
   __syncthreads();
+  pdl_trigger();
   int chunks = 0, before = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {

@@ -87,3 +87,29 @@ def test_a_prompt_of_thousands_of_rows(fmt, hq, hk, d, rows):
     assert not got[0].any()
     _near(got, _exact(q, kc, vc, req, ends, table, page, d ** -0.5))
     native.check_errors()
+
+
+@pytest.mark.parametrize("hk,d,keys", [(1, 64, 50), (1, 256, 100), (8, 128, 3000)])
+def test_between_projections(hk, d, keys):
+    """GEMMs right before and after, which hold tensor memory too and start before their predecessor ends."""
+    from eagle4_b200.ops import native
+
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    kc, vc = _cache(gen, 4096, hk, d, "fp8")
+    w = [torch.randn(n, k, generator=gen, device="cuda").mul_(0.05).to(torch.bfloat16)
+         for n, k in ((4 * hk * d, 512), (512, 4 * hk * d))]
+    x = torch.randn(1, 512, generator=gen, device="cuda").to(torch.bfloat16)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    args = (torch.arange(256, device="cuda").int()[None], 16, i32(0), i32(0), i32(keys), i32(0)[None], i32(0), d ** -0.5, keys)
+
+    def step():
+        q = ops.linear(x, w[0]).view(1, 4 * hk, d)
+        return ops.linear(ops.attention(q, kc, vc, *args), w[1])
+
+    want = step().clone()
+    torch.cuda.synchronize()
+    for _ in range(100):
+        got = step()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    native.check_errors()
