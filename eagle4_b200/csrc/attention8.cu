@@ -25,10 +25,10 @@
 // and fold each chunk's (maximum, sum, output) into fp32 registers. A (row, kv head) inside one CTA is finished there;
 // one cut by a CTA boundary leaves partials that a small second kernel folds.
 //
-// Bound: HBM for long caches (32 rows of 32768 keys, 8 x 128: 424 us, 5.2 TB/s, 0.80 of the copy rate; one row of 131071
-// keys, 4 x 256 int8: 59 us, 0.71); the softmax warps' instructions, some 2000 cycles a chunk, where rows are short or
-// share their keys through L2 (8 x 16 tree rows over 1900 keys: 126 us); launch and the dependent loads of two kernels
-// for one short row (4096 keys: 14 us). Three digits instead of two cost nothing measurable and keep the
+// Bound: HBM for long caches (32 rows of 32768 keys, 8 x 128: 420 us, 5.3 TB/s, 0.81 of the copy rate; one row of 131071
+// keys, 4 x 256 int8: 58 us, 0.72); the softmax warps' instructions, some 2000 cycles a chunk, where rows are short or
+// share their keys through L2 (8 x 16 tree rows over 1900 keys: 118 us; a prompt of 8192 rows, 4 x 256: 16.8 ms); launch
+// and the dependent loads of two kernels for one short row (4096 keys: 14 us). Three digits instead of two cost nothing measurable and keep the
 // digits' error at or below the rounding of fp16 outputs.
 //
 // A row's result must not depend on its batch: a token decoded alone and the same token verified inside a tree have to
@@ -240,7 +240,7 @@ __host__ __device__ constexpr int smem_bytes(int KB, int NH) {
 }
 // CTAs that share an SM: two need 2 x (dynamic + 2048 static + 1024 reserved) bytes within its 228 KB and 96 registers a
 // thread. With 5 to 8 heads the two fit to the byte and spill some 200 bytes a thread: 32 rows of 32768 keys, 64/8 heads x
-// 128, take 671 us (fp8) and 664 us (int8), one CTA without spills 642 and 768.
+// 128, take 640 us (fp8) and 646 us (int8), one CTA without spills 642 and 768.
 __host__ __device__ constexpr int ctas_per_sm(int KB, int NH) { return KB == 1 && NH <= 8 ? 2 : 1; }
 static_assert(ctas_per_sm(1, 8) * (smem_bytes(1, 8) + 2048 + 1024) <= 228 * 1024, "two CTAs an SM up to 8 heads");
 // S and O accumulators, two of each
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_ke
   __shared__ int s_warp[kThreads / 32], s_at[2][4];  // begin and end: row, head, chunk, position
   __shared__ __align__(16) float red_m[2][4][NH], red_l[2][4][NH], s_qf[NH];
   __shared__ __align__(16) int s_cell[kLoad / 32][32];
-  __shared__ int s_bad;
+  __shared__ int s_bad, s_first;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned char* Vs = smem + NS * KB * kTile;
   unsigned char* Qt = smem + NS * 2 * KB * kTile;
@@ -503,7 +503,12 @@ __global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_ke
   w.h = s_at[0][1];
   w.c = s_at[0][2];
   if (w.r < p.T && w.c == w.n) w.next_head(p);
-  if (tid == 0) p.info[blockIdx.x] = make_int4(w.r, w.h, w.c / w.piece, w.n);
+  if (tid == 0) {
+    p.info[blockIdx.x] = make_int4(w.r, w.h, w.c / w.piece, w.n);
+    // The boundary before CTA b lies at chunk floor(chunks b / grid): the first one past the start of the (row, kv head)
+    // that this CTA begins inside of (read after the softmax warps' first barrier).
+    s_first = w.c ? int((int64_t(s_at[0][3] - w.c + 1) * gridDim.x + chunks - 1) / chunks) - 1 : 0;
+  }
   const int end = s_at[1][3] < 0 ? chunks : s_at[1][3];
   const int count = s_at[0][3] < 0 ? 0 : end - s_at[0][3];  // chunks of this CTA
   for (int r = blockIdx.x; r < p.T; r += gridDim.x)  // rows that see nothing
@@ -666,9 +671,6 @@ __global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_ke
     float m[H], pm[H];  // maxima of this chunk and the one before
     // One step takes chunk i to its weights, then folds the output of chunk i - 1, whose product ran meanwhile.
     Walk f = w;  // the chunk being folded
-    // The boundary before CTA b lies at chunk floor(chunks b / grid): the first one past the start of the (row, kv head)
-    // that this CTA begins inside of.
-    const int first_cut = w.c ? int((int64_t(s_at[0][3] - w.c + 1) * gridDim.x + chunks - 1) / chunks) - 1 : 0;
     for (int i = 0; i <= count; ++i) {
       const int st = i % NS;
       if (i < count) {
@@ -767,7 +769,7 @@ __global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_ke
         if (j == 0 || f.c == 0) {
           s.whole = f.c == 0 && f.n <= count - j;
           s.part = f.c / f.piece;
-          s.region = f.c == 0 ? blockIdx.x : first_cut;
+          s.region = f.c == 0 ? blockIdx.x : s_first;
           s.clear_piece();
           s.clear_row();
         }

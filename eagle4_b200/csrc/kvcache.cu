@@ -5,8 +5,8 @@
 // besides wide accesses is to spend few instructions per element. A cache row (one token's one kv head) is handled by
 // a group of up to 16 lanes of one warp, two pieces of eight elements a lane (the second piece half a row further, so
 // that every access of the group is one run of 16-byte vectors): its RMS and largest magnitude are at most four
-// butterfly shuffles, and what is done once per row (scale, reciprocal, address) is shared by 16 elements. Sums, norms, rotations and scales are fp32; the only roundings below 32 bits are the stored codes or bf16
-// rows. A row's result does not depend on how many rows share the launch.
+// butterfly shuffles, and what is done once per row (scale, reciprocal, address) is shared by 16 elements. Sums, norms,
+// rotations and scales are fp32; the only roundings below 32 bits are the stored codes or bf16 rows. A row's result does not depend on how many rows share the launch.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -566,7 +566,9 @@ torch::Tensor prepare_axes(const torch::Tensor& qkv, const torch::Tensor& pos, c
   p.norm_offset = norm_offset;
   p.eps = float(eps);
   p.inv_d = 1.f / float(D);
-  // a row's heads are spread over several blocks only while the rows alone leave SMs idle
+  // A row's heads are spread over several blocks only while the rows alone leave SMs idle. One block a row / spread, us,
+  // 24/4 x 256 into int8: 1 row 3.8 / 2.9, 128 rows 3.9 / 3.4, 512 6.3 / 6.3, 1024 9.8 / 11.1, 2048 17.6 / 20.5; 32/8 x 128
+  // crosses at the same count.
   const int64_t passes = ceil_div(Hq + 2 * Hk, int64_t(kWarps) * (32 / p.lanes));
   const dim3 grid(T, T >= 512 ? 1 : passes);
   auto st = at::cuda::getCurrentCUDAStream().stream();
