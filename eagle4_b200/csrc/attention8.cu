@@ -250,13 +250,18 @@ __host__ __device__ constexpr int tmem_columns(int KB, int NH) {
   return n;
 }
 
+// A row's context positions, for any two int32 bounds.
+E4_DEV int context_keys(const Args& p, int r) {
+  const int a = p.start[r], b = p.end[r];
+  return b > a ? int(min(uint32_t(b) - uint32_t(a), 0x7fffffffu)) : 0;
+}
 E4_DEV int total_keys(const Args& p, int r) {
-  const int n = max(p.end[r] - p.start[r], 0) + min(max(p.n_extra[r], 0), p.extra_ld);
-  if ((n + kChunk - 1) / kChunk > p.max_chunks) {
+  const uint32_t n = uint32_t(context_keys(p, r)) + uint32_t(min(max(p.n_extra[r], 0), p.extra_ld));
+  if (n > uint32_t(p.max_chunks * kChunk)) {  // (at most 2^31 - 256: checked on the host)
     record_error(p.err, kErrBadShape);
     return p.max_chunks * kChunk;
   }
-  return n;
+  return int(n);
 }
 // Chunks of a piece of a row with ``n`` chunks: its pieces over all kv heads come to about ``spread``.
 E4_DEV int piece_chunks(const Args& p, int n) { return max((n * p.Hk + p.spread - 1) / p.spread, 1); }
@@ -593,7 +598,7 @@ __global__ void __launch_bounds__(num_threads(KB), ctas_per_sm(KB, NH)) attn8_ke
       if (w.r != row) {
         row = w.r;
         c0 = p.start[row];
-        nctx = max(p.end[row] - c0, 0);
+        nctx = context_keys(p, row);
         const int b = p.req[row];
         table = b >= 0 && b < p.bt_rows ? p.bt + int64_t(b) * p.bt_ld : nullptr;
       }
@@ -912,6 +917,7 @@ torch::Tensor attention8(const torch::Tensor& q, const torch::Tensor& kc, const 
   TORCH_CHECK(Hk > 0 && Hq > 0 && Hq % Hk == 0 && Hq / Hk <= 16, "attention: query heads per kv head must be <= 16");
   TORCH_CHECK(slots * Hk < (int64_t(1) << 31), "attention: the cache has too many (slot, kv head) rows");
   TORCH_CHECK(page > 0 && page < (int64_t(1) << 31) && slots > 0 && max_keys >= 0, "attention: empty cache or page");
+  TORCH_CHECK(max_keys <= (int64_t(1) << 31) - 2 * kChunk, "attention: too many keys");
   auto rows = [&](const torch::Tensor& t, const char* name, int64_t dims) {
     TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == dims && t.is_contiguous() && t.device() == dev &&
                     (name[0] == 'b' || t.size(0) == T),

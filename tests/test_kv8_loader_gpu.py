@@ -41,3 +41,28 @@ def test_every_lane_reads_its_own_keys_cell(fmt, hq, hk, d):
     for _ in range(20):
         assert torch.equal(split(), want)
     native.check_errors()
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "int8"])
+def test_lengths_past_the_bound_are_reported(fmt):
+    """A row longer than ``max_keys`` says, up to the largest length an int32 holds: the error word, the other rows as
+    they are, and nothing read past the row's block table."""
+    from eagle4_b200.ops import native
+
+    kc, vc = (new_cache(64, 2, 64, torch.bfloat16, kv_code(fmt), "cuda") for _ in range(2))
+    x = torch.randn(64, 2, 64, device="cuda")
+    ops.kv_write(x, x, torch.arange(64, device="cuda"), kc, vc)
+    q = torch.randn(3, 4, 64, device="cuda").to(torch.bfloat16)
+    call = lambda start, end, keys: ops.attention(q, kc, vc, _i32([[0, 1, 2, 3]]), 16, _i32([0] * 3), _i32(start), _i32(end),  # noqa: E731
+                                                  _i32([[0]] * 3), _i32([0] * 3), 0.1, keys)
+    want = call([0, 0, 0], [50, 0, 17], 64)
+    native.check_errors()
+    top = 2 ** 31 - 1
+    for start, end in ((0, top), (-top, top), (-top - 1, 5), (0, 300)):
+        got = call([0, start, 0], [50, end, 17], 64)
+        with pytest.raises(RuntimeError, match="error code"):
+            native.check_errors()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
+    with pytest.raises(RuntimeError, match="too many keys"):
+        call([0] * 3, [1] * 3, 2 ** 31)
+    native.check_errors()
